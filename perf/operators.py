@@ -14,7 +14,6 @@ The operators:
 * gated RMS norm over groups of the last dimension: norm(x * silu(z)) * w, or norm(x) * w * silu(z).
 """
 
-import functools
 import math
 import os
 import sys
@@ -174,8 +173,7 @@ _EPS = 1e-5
 # ---- the framework's calls ---------------------------------------------------------------------
 
 
-@functools.lru_cache(None)
-def _package():  # once, as a program imports it
+def _package():
     root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mamba-cpu_b200")
     if root not in sys.path:
         sys.path.insert(0, root)
