@@ -701,6 +701,8 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const NormArgs a, const 
 
 // ---- launch: pick the instantiation -----------------------------------------------------------
 
+constexpr int kMostShared = 208 * 1024;  // of an SM's 227 KB, for the copies of the CTAs that it holds
+
 template <typename T, typename TR, int GATE, bool BWD, int K, int MAXT, int EDGES>
 cudaError_t norm_run(const NormArgs& a, const NormShape& s, cudaStream_t stream) {
   using Types = NormTypes<T, TR, GATE>;
@@ -721,12 +723,17 @@ cudaError_t norm_run(const NormArgs& a, const NormShape& s, cudaStream_t stream)
   const size_t row_ahead = (size_t)units * 16 * s.threads * s.resident;
   const bool shallow = Types::kRes && (BWD ? row_ahead >= 56 * 1024 || (K == 1 && s.tpr <= 64) : row_ahead >= 26 * 1024);
   int stages = shallow ? 2 : 3;
-  while (stages > 1 && (stages * stage + sigmoids) * s.resident > 208 * 1024) --stages;
+  while (stages > 1 && (stages * stage + sigmoids) * s.resident > kMostShared) --stages;
   const int teams = s.threads / s.tpr;
   const size_t fold = BWD && teams > 1 ? sizeof(float) * (a.want_db ? 2 : 1) * teams * (size_t)a.n : 0;
   const size_t smem = stages * stage + sigmoids > fold ? stages * stage + sigmoids : fold;
+  // The leave is one number, whatever this call takes: another thread that launches the kernel at another width between
+  // these lines and the launch must not lower it.
+  static_assert((size_t)(units + (EDGES == 2 ? K * tensors : 0)) * 16 * MAXT +
+                        (BWD && Types::kGated && keep_sigmoids<MAXT> ? (size_t)K * 2 * 16 * MAXT : 0) <= kMostShared,
+                "a stage of the widest rows");
   if (smem > 40 * 1024) {  // 48 KB, the kernel's own arrays among them, need no leave
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared);
     if (e != cudaSuccess) return e;
   }
   if (!BWD && grid.x > 1) {

@@ -14,6 +14,7 @@ import torch
 
 import block_oracles as bo
 import mamba_cpu_b200 as mb
+from mamba_cpu_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -351,6 +352,46 @@ def test_streams_and_threads():
     [t.join() for t in threads]
     for r, g in zip(ref, got):
         assert all(torch.equal(a, b) for a, b in zip(r, g))
+
+
+def test_threads_with_different_widths():
+    """Calls of one kernel at widths that ask for different amounts of shared memory, from two threads at once through
+    the C ABI (which leaves the interpreter's lock alone): every one is launched with what it asked for."""
+    def forward(n):
+        x, z, w = (rand(r, n, dtype=BF16, seed=r + k).cuda() for k, r in enumerate((4, 4, 1)))
+        out = torch.empty_like(x)
+        p = _lib.NormParams(x=x.data_ptr(), z=z.data_ptr(), weight=w.data_ptr(), out=out.data_ptr(), rows=4, dim=n,
+                            group_size=n, eps=1e-5, io_dtype=_lib.BF16, residual_dtype=_lib.BF16, weight_dtype=_lib.BF16,
+                            rms=1, gate=_lib.GATE_BEFORE_NORM)
+        return lambda s: _lib.lib.mb200_norm_fwd(p, s), out, mb.gated_rms_norm_fn(x, z, w[0]), (x, z, w)
+
+    def backward(n):
+        dy, s, w = rand(4, n, dtype=BF16).cuda(), rand(4, n, seed=1).cuda(), rand(n, seed=2).cuda()
+        dx, dw = torch.empty_like(dy), torch.empty_like(w)
+        f = _lib.NormParams(x=s.data_ptr(), residual=s.data_ptr(), weight=w.data_ptr(), rows=4, dim=n, group_size=n,
+                            eps=1e-5, io_dtype=_lib.BF16, rms=1)
+        p = _lib.NormBwdParams(fwd=f, dout=dy.data_ptr(), dx=dx.data_ptr(), dweight=dw.data_ptr())
+        ref = torch.ops.mamba_b200.norm_bwd(dy, None, s, None, w, F32, None, 1e-5, n, True, 0, False)[0]
+        size = _lib.lib.mb200_norm_bwd_workspace_size(p)
+        ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+        return lambda st: _lib.lib.mb200_norm_bwd(p, ws.data_ptr(), size, st), dx, ref, (dy, s, w, dw, ws)
+
+    for make, widths in ((forward, (4096, 5120)), (backward, (512, 1024))):
+        cases = [make(n) for n in widths]
+        torch.cuda.synchronize()
+        refused = [0, 0]
+
+        def work(k):
+            stream = torch.cuda.Stream()
+            for _ in range(20000):
+                refused[k] += cases[k][0](stream.cuda_stream) != 0
+            stream.synchronize()
+
+        threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+        [t.start() for t in threads]
+        [t.join() for t in threads]
+        assert refused == [0, 0], f"{make.__name__}: launches refused {refused}"
+        assert all(torch.equal(out, ref) for _, out, ref, _ in cases)
 
 
 def test_first_order_only():
