@@ -93,6 +93,17 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
+
+// Nothing here has a forward-mode derivative. A tangent that the kernels passed over would come back as zero.
+void no_tangents(std::initializer_list<const Tensor*> ts, std::initializer_list<const OptTensor*> more) {
+  const auto check = [](const Tensor& t) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(),
+                                "forward-mode derivatives are not supported by mamba_cpu_b200");
+  };
+  for (const Tensor* t : ts) check(*t);
+  for (const OptTensor* t : more)
+    if (t->has_value()) check(**t);
+}
 Tensor or_undefined(const OptTensor& t) { return given(t) ? *t : Tensor(); }
 
 // ---- gated linear recurrence ----------------------------------------------------------------------
@@ -239,6 +250,7 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& u, const Tensor& decay_gate,
   want_shape("A", A, {d}, u, "u");
   want_shape("initial_state", initial_state, {b, d}, u, "u");
   want_shape("seq_idx", seq_idx, {b, l}, u, "u");
+  no_tangents({&u, &decay_gate, &input_gate, &A}, {&initial_state});
   TORCH_CHECK_NOT_IMPLEMENTED(!A.is_complex(), "complex A is not supported yet");
   TORCH_CHECK_TYPE(!given(seq_idx) || at::isIntegralType(seq_idx->scalar_type(), /*includeBool=*/false),
                    "seq_idx must hold integers, got ", seq_idx->scalar_type());
@@ -343,6 +355,7 @@ Tensor gated_step(Tensor state, const Tensor& u, const Tensor& decay_gate, const
   want_shape("input_gate", input_gate, u.sizes(), u, "u");
   want_shape("A", A, {d}, u, "u");
   want_shape("out_state", out_state, u.sizes(), u, "u");
+  no_tangents({&state, &u, &decay_gate, &input_gate, &A}, {&out_state});
   TORCH_CHECK_NOT_IMPLEMENTED(!A.is_complex(), "complex A is not supported yet");
   const bool apart = given(out_state) && !out_state->is_same(state);
   Tensor target = apart ? *out_state : state;
@@ -609,6 +622,7 @@ std::tuple<Tensor, Tensor> norm(const Tensor& x, const OptTensor& weight, const 
   want_shape("weight", weight, {dim}, x, "x");
   want_shape("bias", bias, {dim}, x, "x");
   want_shape("residual", residual, x.sizes(), x, "x");
+  no_tangents({&x}, {&weight, &bias, &residual});
   TORCH_CHECK_NOT_IMPLEMENTED(dim <= MB200_NORM_MAX_DIM, "a last dimension > ", MB200_NORM_MAX_DIM,
                               " is not supported by the B200 kernels");
   TORCH_CHECK_VALUE(eps >= 0, "eps must not be negative, got ", eps);
@@ -640,6 +654,7 @@ Tensor gated_norm(const Tensor& x, const Tensor& z, const OptTensor& weight, dou
   const int64_t dim = x.size(-1);
   want_shape("z", z, x.sizes(), x, "x");
   want_shape("weight", weight, {dim}, x, "x");
+  no_tangents({&x, &z}, {&weight});
   const int64_t group = group_size.value_or(dim);
   TORCH_CHECK_VALUE(dim == 0 || (group >= 1 && dim % group == 0), "group_size must divide the last dimension ", dim,
                     ", got ", group);

@@ -7,8 +7,9 @@ operator; it stands beside ``selective_scan_fn``, whose (batch, dim, seqlen) lay
     h_t = a_t h_{t-1} + sqrt(1 - a_t^2) * sigmoid(input_gate_t) * u_t,     y_t = h_t
 
 The gates, the root and the recurrence run in one kernel (``mb200_gated_scan_fwd`` /
-``mb200_gated_scan_bwd`` in libmamba_b200.so), in float32 for every input dtype. Argument checks and
-the autograd node are those of ``mamba_b200::gated_scan`` / ``::gated_step`` (csrc/torch_ops.cpp).
+``mb200_gated_scan_bwd`` in libmamba_b200.so), in float32 for every input dtype. Gradients are reverse
+mode: a forward-mode tangent on any argument raises ``NotImplementedError``. Argument checks and the
+autograd node are those of ``mamba_b200::gated_scan`` / ``::gated_step`` (csrc/torch_ops.cpp).
 """
 
 import torch

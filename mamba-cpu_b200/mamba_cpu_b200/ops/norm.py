@@ -4,7 +4,8 @@ The norms around a mixer: ``layer_norm_fn`` / ``rms_norm_fn`` before it, on the 
 ``gated_rms_norm_fn`` behind its scan. The mamba-cpu reference leaves them to PyTorch; here each is
 one kernel forward and one (plus the reduction of the weight's gradient over the rows) backward,
 ``mb200_norm_fwd`` / ``mb200_norm_bwd`` in libmamba_b200.so. Arithmetic is float32 for every input
-dtype. Argument checks and the autograd nodes are those of ``mamba_b200::norm`` / ``::gated_norm``
+dtype. Gradients are reverse mode: a forward-mode tangent on any argument raises ``NotImplementedError``.
+Argument checks and the autograd nodes are those of ``mamba_b200::norm`` / ``::gated_norm``
 (csrc/torch_ops.cpp).
 """
 

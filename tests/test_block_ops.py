@@ -10,6 +10,7 @@ import tempfile
 import numpy as np
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 import block_oracles as bo
@@ -259,6 +260,39 @@ def test_shapes_and_dtypes_on_fake_tensors():
         assert y.grad_fn is not None and y.shape == x.shape
         got = ops.norm_bwd(y.detach(), None, x.detach(), x.detach(), w.detach(), None, None, 1e-5, 4, True, 1, False)
         assert [t.shape for t in got] == [x.shape, (0,), x.shape, (16,), (0,)]
+
+
+_TENSORS = {  # every tensor argument by name, and the call
+    "scan": (dict(u=(2, 4, 8), r=(2, 4, 8), i=(2, 4, 8), A=(4,), h0=(2, 4)),
+             lambda t: mb.gated_linear_scan_fn(t["u"], t["r"], t["i"], t["A"], t["h0"])),
+    "step": (dict(state=(2, 4), u=(2, 4), r=(2, 4), i=(2, 4), A=(4,)),
+             lambda t: mb.gated_linear_scan_update(t["state"], t["u"], t["r"], t["i"], t["A"])),
+    "step to": (dict(state=(2, 4), u=(2, 4), out_state=(2, 4), A=(4,)),
+                lambda t: mb.gated_linear_scan_update(t["state"], t["u"], t["u"], t["u"], t["A"], t["out_state"])),
+    "layer norm": (dict(x=(3, 8), w=(8,), b=(8,), res=(3, 8)),
+                   lambda t: mb.layer_norm_fn(t["x"], t["w"], t["b"], t["res"])),
+    "rms norm": (dict(x=(3, 8), w=(8,), b=(8,), res=(3, 8)),
+                 lambda t: mb.rms_norm_fn(t["x"], t["w"], t["b"], t["res"], prenorm=True)[1]),
+    "gated norm": (dict(x=(3, 8), z=(3, 8), w=(8,)), lambda t: mb.gated_rms_norm_fn(t["x"], t["z"], t["w"])),
+}
+
+
+@pytest.mark.parametrize("name,arg", [(n, a) for n, (shapes, _) in _TENSORS.items() for a in shapes])
+def test_forward_mode_is_refused(name, arg):
+    """A tangent on any argument raises, with gradients enabled or not: none comes back as zero."""
+    shapes, call = _TENSORS[name]
+    with FakeTensorMode():
+        t = {k: _fake(*s) for k, s in shapes.items()}
+        direction = _fake(*shapes[arg])
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                with fwAD.dual_level():
+                    with pytest.raises(NotImplementedError, match="forward-mode"):
+                        call({**t, arg: fwAD.make_dual(t[arg], direction)})
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    torch.func.jvp(lambda v: call({**t, arg: v}), (t[arg],), (direction,))
+        with fwAD.dual_level():  # no argument has one
+            call(t)
 
 
 # ---- the oracles' gradients against differences ---------------------------------------------------------
