@@ -99,9 +99,14 @@ def mamba_inner_fn(xz, conv1d_weight, conv1d_bias, x_proj_weight, delta_proj_wei
     d_inner = x.shape[1]
     x_dbl = F.linear(x.transpose(1, 2).reshape(batch * seqlen, d_inner), x_proj_weight)  # (b l, r + 2n)
     # delta as (d, b l): its (b, d, l) view below is seqlen-contiguous, which the scan reads in place
-    delta = delta_proj_weight @ x_dbl[:, :dt_rank].t()
-    if dt_rms_weight is not None:
-        delta = _rms_norm(delta.t(), dt_rms_weight, b_c_dt_rms_eps).t()  # over d_inner
+    if dt_rms_weight is None:
+        delta = delta_proj_weight @ x_dbl[:, :dt_rank].t()
+    else:
+        # The norm over d_inner goes along (b l, d) rows, as the projection gives them here; one transposing copy
+        # follows. d_inner 8192, 4 x 2048 steps, bf16: this body 2.16 ms forward, 7.02 with gradients; with the norm of
+        # the transposed projection (a copy before and one behind it) 2.42 and 7.55, with it in plain PyTorch 2.59 and 8.77.
+        delta = _rms_norm(F.linear(x_dbl[:, :dt_rank], delta_proj_weight), dt_rms_weight, b_c_dt_rms_eps)
+        delta = delta.t().contiguous()
     delta = delta.reshape(d_inner, batch, seqlen).transpose(0, 1)  # (b, d, l)
 
     def _bc(M, start, bias, rms_w):

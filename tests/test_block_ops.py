@@ -262,6 +262,30 @@ def test_shapes_and_dtypes_on_fake_tensors():
         assert [t.shape for t in got] == [x.shape, (0,), x.shape, (16,), (0,)]
 
 
+@pytest.mark.parametrize("rms", [False, True])
+@pytest.mark.parametrize("b,l", [(1, 12), (3, 12)])
+def test_mixer_delta_is_read_in_place(monkeypatch, rms, b, l):
+    """mamba_inner_fn hands the scan a delta whose (b, d, l) view has contiguous rows, with delta's norm and without."""
+    from mamba_cpu_b200 import hf
+
+    d, n, r, dm, seen = 32, 4, 2, 16, []
+
+    def scan(u, delta, *rest):
+        seen.append(delta)
+        return u
+
+    monkeypatch.setattr(hf, "causal_conv1d_fn", lambda x, w, bias, activation: x.contiguous())
+    monkeypatch.setattr(hf, "selective_scan_fn", scan)
+    bf = torch.bfloat16
+    with FakeTensorMode():
+        y = hf.mamba_inner_fn(_fake(b, 2 * d, l, dtype=bf), _fake(d, 1, 4, dtype=bf), None, _fake(r + 2 * n, d, dtype=bf),
+                              _fake(d, r, dtype=bf), _fake(dm, d, dtype=bf), None, _fake(d, n),
+                              dt_rms_weight=_fake(d, dtype=bf) if rms else None)
+    delta, = seen
+    assert y.shape == (b, l, dm) and delta.shape == (b, d, l) and delta.dtype == bf
+    assert delta.stride()[1:] == (b * l, 1) and (b == 1 or delta.stride(0) == l)
+
+
 _TENSORS = {  # every tensor argument by name, and the call
     "scan": (dict(u=(2, 4, 8), r=(2, 4, 8), i=(2, 4, 8), A=(4,), h0=(2, 4)),
              lambda t: mb.gated_linear_scan_fn(t["u"], t["r"], t["i"], t["A"], t["h0"])),
