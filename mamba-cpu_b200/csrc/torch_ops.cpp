@@ -479,7 +479,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> norm_bwd(const Tensor& dout, 
                                                             std::optional<at::ScalarType> residual_type,
                                                             std::optional<at::ScalarType> bias_type, double eps,
                                                             int64_t group, bool rms, int64_t gate,
-                                                            bool want_dresidual) {
+                                                            bool want_dresidual, bool want_dweight) {
   constexpr const char* name = "mamba_b200::norm_bwd";
   const auto io = dout.scalar_type();
   want_device({&dout, &rows}, {&dsum, &z, &weight}, name);
@@ -512,14 +512,15 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> norm_bwd(const Tensor& dout, 
   Tensor dx = make(dout.sizes(), dout, io);
   Tensor dres = maybe(own_dres, dout.sizes(), own_dres ? *residual_type : io);
   Tensor dz = maybe(given(z), dout.sizes(), io);
-  Tensor dw = maybe(given(weight), {dim}, given(weight) ? w_type : io);
+  const bool want_dw = given(weight) && want_dweight;
+  Tensor dw = maybe(want_dw, {dim}, want_dw ? w_type : io);
   Tensor db = maybe(bias_type.has_value(), {dim}, bias_type.value_or(io));
   p.dout = ptr(dout);
   p.dsum = ptr(dsum);
   p.dx = ptr(dx);
   p.dresidual = own_dres ? ptr(dres) : nullptr;
   p.dz = given(z) ? ptr(dz) : nullptr;
-  p.dweight = given(weight) ? ptr(dw) : nullptr;
+  p.dweight = want_dw ? ptr(dw) : nullptr;
   p.dbias = bias_type ? ptr(db) : nullptr;
   const auto bytes = static_cast<int64_t>(mb200_norm_bwd_workspace_size(&p));
   Tensor ws = bytes > 0 ? make({bytes}, dout, at::kByte) : Tensor();
@@ -545,7 +546,8 @@ struct Norm : torch::autograd::Function<Norm> {
     ctx->saved_data["f"] = std::vector<int64_t>{
         res ? static_cast<int64_t>(residual->scalar_type()) : -1,
         given(bias) && bias->requires_grad() ? static_cast<int64_t>(bias->scalar_type()) : -1,
-        static_cast<int64_t>(x.scalar_type()), rms, res && residual->requires_grad()};
+        static_cast<int64_t>(x.scalar_type()), rms, res && residual->requires_grad(),
+        given(weight) && weight->requires_grad()};
     ctx->saved_data["eps"] = eps;
     at::AutoDispatchBelowADInplaceOrView below;
     auto [out, total] = norm_fwd_op().call(x, residual, std::nullopt, weight, bias, eps, x.size(-1), rms,
@@ -571,10 +573,10 @@ struct Norm : torch::autograd::Function<Norm> {
     auto [dx, dres, dz, dw, db] =
         norm_bwd_op().call(dout, ds, s[0], std::nullopt, s[1].defined() ? OptTensor(s[1]) : std::nullopt, type(f[0]),
                            type(f[1]), ctx->saved_data["eps"].toDouble(), s[0].size(-1), f[3] != 0, MB200_GATE_NONE,
-                           f[4] != 0);
+                           f[4] != 0, f[5] != 0);
     none[0] = dx;
     if (f[4]) none[1] = *type(f[0]) == io ? dx : dres;
-    if (s[1].defined()) none[2] = dw;
+    if (f[5]) none[2] = dw;
     if (f[1] >= 0) none[3] = db;
     return none;
   }
@@ -586,7 +588,7 @@ struct GatedNorm : torch::autograd::Function<GatedNorm> {
     at::AutoDispatchBelowADInplaceOrView below;
     auto [out, total] = norm_fwd_op().call(x, std::nullopt, z, weight, std::nullopt, eps, group, true, gate, false);
     ctx->save_for_backward({x, z, or_undefined(weight)});
-    ctx->saved_data["f"] = std::vector<int64_t>{group, gate};
+    ctx->saved_data["f"] = std::vector<int64_t>{group, gate, given(weight) && weight->requires_grad()};
     ctx->saved_data["eps"] = eps;
     ctx->set_materialize_grads(false);
     return {out};
@@ -600,9 +602,9 @@ struct GatedNorm : torch::autograd::Function<GatedNorm> {
     auto [dx, dres, dz, dw, db] =
         norm_bwd_op().call(grads[0].contiguous(), std::nullopt, s[0], s[1],
                            s[2].defined() ? OptTensor(s[2]) : std::nullopt, std::nullopt, std::nullopt,
-                           ctx->saved_data["eps"].toDouble(), f[0], true, f[1], false);
+                           ctx->saved_data["eps"].toDouble(), f[0], true, f[1], false, f[2] != 0);
     none[0] = dx, none[1] = dz;
-    if (s[2].defined()) none[2] = dw;
+    if (f[2]) none[2] = dw;
     return none;
   }
 };
@@ -692,7 +694,8 @@ TORCH_LIBRARY_FRAGMENT(mamba_b200, m) {
       "bool rms, int gate, bool want_sum) -> (Tensor, Tensor)");
   m.def(
       "norm_bwd(Tensor dout, Tensor? dsum, Tensor rows, Tensor? z, Tensor? weight, ScalarType? residual_dtype, "
-      "ScalarType? bias_dtype, float eps, int group_size, bool rms, int gate, bool want_dresidual) "
+      "ScalarType? bias_dtype, float eps, int group_size, bool rms, int gate, bool want_dresidual, "
+      "bool want_dweight=True) "
       "-> (Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def(
       "gated_scan(Tensor u, Tensor decay_gate, Tensor input_gate, Tensor A, Tensor? initial_state, Tensor? seq_idx) "

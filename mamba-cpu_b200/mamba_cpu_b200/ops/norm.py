@@ -24,13 +24,15 @@ def _(x, residual, z, weight, bias, eps, group_size, rms, gate, want_sum):
 
 
 @torch.library.register_fake("mamba_b200::norm_bwd")
-def _(dout, dsum, rows, z, weight, residual_dtype, bias_dtype, eps, group_size, rms, gate, want_dresidual):
+def _(dout, dsum, rows, z, weight, residual_dtype, bias_dtype, eps, group_size, rms, gate, want_dresidual,
+      want_dweight=True):
     dim, io = dout.shape[-1:], dout.dtype
     own_dres = want_dresidual and residual_dtype is not None and residual_dtype != io
+    own_dw = weight is not None and want_dweight
     return (dout.new_empty(dout.shape),
             dout.new_empty(dout.shape if own_dres else (0,), dtype=residual_dtype if own_dres else io),
             dout.new_empty(dout.shape if z is not None else (0,)),
-            dout.new_empty(dim if weight is not None else (0,), dtype=weight.dtype if weight is not None else io),
+            dout.new_empty(dim if own_dw else (0,), dtype=weight.dtype if own_dw else io),
             dout.new_empty(dim if bias_dtype is not None else (0,), dtype=bias_dtype or io))
 
 

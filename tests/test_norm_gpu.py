@@ -394,6 +394,36 @@ def test_threads_with_different_widths():
         assert all(torch.equal(out, ref) for _, out, ref, _ in cases)
 
 
+@pytest.mark.parametrize("rows", [3, 700])
+def test_frozen_weight(rows):
+    """A weight that asks for no gradient gets no sums over the rows; the other gradients are the same."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Sums(TorchDispatchMode):  # sizes of dweight and dbias of the backward calls
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            if func is torch.ops.mamba_b200.norm_bwd.default:
+                self.seen.append((out[3].numel(), out[4].numel()))
+            return out
+
+    n = 200
+    x, z, dy = (rand(rows, n, dtype=BF16, seed=k).cuda() for k in range(3))
+    w, b = rand(n, seed=3).cuda(), rand(n, seed=4).cuda()
+    calls = [(lambda x, w, b: mb.layer_norm_fn(x, w, b, residual=z), True), (lambda x, w, b: mb.rms_norm_fn(x, w), False),
+             (lambda x, w, b: mb.gated_rms_norm_fn(x, z, w), False)]
+    for call, biased in calls:
+        all_of = [t.clone().requires_grad_() for t in ((x, w, b) if biased else (x, w))]
+        want = torch.autograd.grad(call(*(all_of + [b])[:3]), all_of, dy)
+        for wants_b in ((False, True) if biased else (False,)):
+            xl, bl = x.clone().requires_grad_(), b.clone().requires_grad_(wants_b)
+            y = call(xl, w, bl)
+            with Sums() as mode:
+                mode.seen = []
+                got = torch.autograd.grad(y, [xl, bl] if wants_b else [xl], dy)
+            assert mode.seen == [(0, n if wants_b else 0)]
+            assert torch.equal(got[0], want[0]) and (not wants_b or torch.equal(got[1], want[2]))
+
+
 def test_first_order_only():
     """Gradients that are asked to be differentiable come, and raise when they are differentiated."""
     x, w, dy = rand(5, 40).cuda().requires_grad_(), rand(40, seed=1).cuda(), rand(5, 40, seed=2).cuda()
