@@ -541,7 +541,7 @@ auto& norm_bwd_op() {
 
 struct Norm : torch::autograd::Function<Norm> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual,
-                               const OptTensor& weight, const OptTensor& bias, double eps, bool rms, bool prenorm) {
+                               const OptTensor& weight, const OptTensor& bias, double eps, bool rms) {
     const bool res = given(residual);
     ctx->saved_data["f"] = std::vector<int64_t>{
         res ? static_cast<int64_t>(residual->scalar_type()) : -1,
@@ -552,14 +552,16 @@ struct Norm : torch::autograd::Function<Norm> {
     at::AutoDispatchBelowADInplaceOrView below;
     auto [out, total] = norm_fwd_op().call(x, residual, std::nullopt, weight, bias, eps, x.size(-1), rms,
                                            MB200_GATE_NONE, res);
+    // The sum is an output whether or not the caller takes it: as one it is saved with its way back to x and the
+    // residual, on which a second backward raises.
     ctx->save_for_backward({res ? total : x, or_undefined(weight)});
     ctx->set_materialize_grads(false);
-    if (prenorm) return {out, total};
+    if (res) return {out, total};
     return {out};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    variable_list none(7);
+    variable_list none(6);
     const Tensor dsum = grads.size() > 1 ? grads[1] : Tensor();
     if (!grads[0].defined() && !dsum.defined()) return none;
     const auto s = ctx->get_saved_variables();
@@ -638,7 +640,7 @@ std::tuple<Tensor, Tensor> norm(const Tensor& x, const OptTensor& weight, const 
   const bool carried = prenorm && res.has_value();
   Tensor out, total;
   if (wants_grad({&xk}) || (res && wants_grad({&*res})) || (w && wants_grad({&*w})) || (b && wants_grad({&*b}))) {
-    auto r = Norm::apply(xk, res, w, b, eps, rms, carried);
+    auto r = Norm::apply(xk, res, w, b, eps, rms);
     out = r[0];
     if (carried) total = r[1];
   } else {

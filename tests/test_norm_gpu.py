@@ -435,6 +435,22 @@ def test_first_order_only():
                 torch.autograd.grad(g.sum(), x)
 
 
+@pytest.mark.parametrize("call", ["layer", "rms", "gated"])
+def test_second_backward_raises(call):
+    """A gradient that was asked to be differentiable says so, and differentiating it raises, whichever input it is of."""
+    x, w, b, z, dy = (t.cuda() for t in (rand(5, 40), rand(40, seed=1), rand(40, seed=2), rand(5, 40, seed=3), rand(5, 40, seed=4)))
+    leaves = [t.requires_grad_() for t in ((x, z, w) if call == "gated" else (x, z, w, b))]
+    if call == "gated":
+        y = mb.gated_rms_norm_fn(x, z, w)
+    else:
+        y = (mb.layer_norm_fn if call == "layer" else mb.rms_norm_fn)(x, w, b, z)
+    grads = torch.autograd.grad(y, leaves, dy, create_graph=True)
+    for g in grads:
+        assert g.requires_grad
+        with pytest.raises(RuntimeError, match="norm_bwd is not implemented"):
+            torch.autograd.grad(g.sum(), x, retain_graph=True)
+
+
 def test_compiled():
     """Traced and run by torch.compile's eager backend, gradients included."""
     x, r, z = (rand(6, 64, seed=k).cuda().requires_grad_() for k in range(3))
