@@ -418,6 +418,17 @@ def test_first_order_only():
             torch.autograd.grad(g.sum(), leaf)
 
 
+def test_second_backward_raises():
+    """A gradient that was asked to be differentiable says so, and differentiating it raises, whichever input it is of."""
+    x = cuda(make(2, 3, 20, F32, initial=True))
+    leaves = [x[k].requires_grad_() for k in NAMES]
+    y = mb.gated_linear_scan_fn(*leaves)
+    for g in torch.autograd.grad(y, leaves, x["dy"], create_graph=True):
+        assert g.requires_grad
+        with pytest.raises(RuntimeError, match="gated_scan_bwd is not implemented"):
+            torch.autograd.grad(g.sum(), leaves[0], retain_graph=True)
+
+
 def test_compiled():
     """Traced and run by torch.compile's eager backend: forward, gradients and the step."""
     x = cuda(make(2, 6, 300, F32, initial=True, packed=True))
