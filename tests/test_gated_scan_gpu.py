@@ -189,6 +189,34 @@ def test_extreme_gates(dtype):
     assert torch.equal(got[1][0, 0], x["h0"][0, 0].cuda())
 
 
+def test_long_memory():
+    """Channels that forget next to nothing: |A| of 0.005 to 0.01 and decay gates around -8, 1 - a of 1e-6 to 6e-6.
+
+    A step's decay is off by half a float32 step below 1, 2^-25: half a unit of 2^-24. Over a chunk of 256 steps a state
+    takes 256 of those halves; its lane's 8 compositions, the 5 joins of the lanes and 5 of the warps round a partial sum
+    (at most twice the largest state, as what two states differ by) and a product of decays: 18 (2 + 1), and 6 for the way
+    in, 60. Inputs are off by 16 units each, decay gates by 12 of 1 - a. The recurrence of the gradients is the same from
+    the other end; du's factors take 30 more."""
+    d, L = 6, 4000
+    x = make(1, d, L, seed=21, initial=True)
+    x["A"] = -torch.linspace(0.005, 0.01, d)
+    x["r"] = x["r"] * 0.25 - 8
+    got, grads = run(x)
+    ref = want(x)
+    s_r, s_i = bo.sigmoid(bo.f64(x["r"])), bo.sigmoid(bo.f64(x["i"]))
+    la = bo.f64(x["A"])[None, :, None] * s_r
+    ms = np.sqrt(-np.expm1(2 * la)) * s_i
+    assert 1e-7 < -la.max() and -la.min() < 1e-5
+    own = 60 * (L // 256 + 2) + L / 2 + 12 * float(-la.sum(-1).min())
+    top = max(np.abs(ref["out"]).max(), np.abs(bo.f64(x["h0"])).max())
+    units = own + 16 * np.abs(ms * bo.f64(x["u"])).sum(-1).max() / top
+    bo.check(got[0], ref["out"], F32, units, scale=top, name="out")
+    bo.check(got[1], ref["last"], F32, units, scale=top, name="last_state")
+    big = max(np.abs(ref["du"] / ms).max(), np.abs(bo.f64(x["dlast"])).max())  # the largest gradient of a state
+    bo.check(grads["h0"], ref["dh0"], F32, own, scale=big, name="dh0")
+    bo.check(grads["u"], ref["du"], F32, own + 30, scale=big * ms.max(), name="du")
+
+
 def test_positive_A_is_nan():
     x = make(1, 2, 9, F32)
     x["A"][1] = 0.5
