@@ -781,7 +781,7 @@ cudaError_t launch_rows(F kernel, const GatedScanArgs& a, int warps, int ctas, c
     // is used), so that the second wave is not left to a few warps. Forward of 1 x 5120 x 65536 bf16, 35 rows
     // an SM: 516 us at 32 at a time, 478 at 23, 456 at 20, 483 at 18. (Rows of 2,048 steps, which are many
     // where they matter, are best left alone: 85 us at 32 at a time, 91 at 20. So is the backward, which
-    // registers hold to 24: 818 us, 820 at 20.)
+    // registers (85 to 92 a thread) hold to 20 anyway.)
     const int64_t per_sm = (rows + sm_count() - 1) / sm_count(), fewer = (per_sm + 1) / 2 + 2;
     if (per_sm > kMostCtas && fewer < kMostCtas) {
       constexpr int kIds = IDS ? kStages<T, IDS> * kIdSlot * (int)sizeof(int32_t) : 0;
