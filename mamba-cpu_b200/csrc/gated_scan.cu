@@ -765,8 +765,12 @@ void row_split(const GatedScanArgs& a, int* warps, int* ctas) {
   *warps = w;
 }
 
-constexpr int kLongRow = 32;    // chunks
-constexpr int kMostCtas = 32;   // that an SM holds
+constexpr int kLongRow = 32;  // chunks
+// One-warp forward CTAs without ids that an SM holds (32 is its most; float32 rows take 7.5 KB of shared memory each),
+// and the most rows an SM of which a second wave is small enough to be evened out.
+template <typename T>
+constexpr int kMostCtas = sizeof(T) == 4 ? 29 : 32;
+constexpr int kMostEvened = 45;
 constexpr int kSmSharedBytes = 228 * 1024, kCtaSharedBytes = 1024;  // of an SM; taken by a CTA besides its request
 
 template <typename T, bool IDS, int TENSORS, int NT, typename F>
@@ -776,16 +780,18 @@ cudaError_t launch_rows(F kernel, const GatedScanArgs& a, int warps, int ctas, c
   cfg.blockDim = dim3(32 * warps / ctas);
   cfg.gridDim = dim3((unsigned)(rows * ctas));
   cfg.dynamicSmemBytes = kStages<T, IDS> * TENSORS * kTensorBytes<T, NT>;  // 32 KB at most
-  if (TENSORS == 3 && warps == 1 && a.chunks >= kLongRow) {
-    // Long rows in a full and a nearly empty wave: fewer at a time (by asking for more shared memory than
-    // is used), so that the second wave is not left to a few warps. Forward of 1 x 5120 x 65536 bf16, 35 rows
-    // an SM: 516 us at 32 at a time, 478 at 23, 456 at 20, 483 at 18. (Rows of 2,048 steps, which are many
-    // where they matter, are best left alone: 85 us at 32 at a time, 91 at 20. So is the backward, which
-    // registers (85 to 92 a thread) hold to 20 anyway.)
+  if (TENSORS == 3 && !IDS && warps == 1 && a.chunks >= kLongRow) {
+    // Long rows in a full and a nearly empty wave: fewer at a time (by asking for more shared memory than is used), so
+    // that the second wave is not left to a few warps. Forward of 1 x 5120 x 65536 bf16, 35 rows an SM: 492 us at 32 at a
+    // time, 461 at 20. Rows of 16,384 steps, us as many at a time as fit and evened out, by rows an SM:
+    //   bf16     33  119 119   35  128 121   38  138 134   40  140 140   42  140 142   44  148 144   46  150 154   56  175 183
+    //   float32  30  191 185   33  220 203   35  257 210   38  259 222   40  267 250   44  279 271   46  283 283   48  285 289
+    // Packed rows, which registers hold to 25, lose (bf16 1 x 5120 x 65536 568 and 578, float32 1 x 5120 x 32768 431 and
+    // 446), and so do rows of 2,048 steps (8 x 4096 x 2048 bf16 85 us at 32 at a time, 91 at 20). Registers (85 to 92 a
+    // thread) hold the backward to 20 rows an SM anyway.
     const int64_t per_sm = (rows + sm_count() - 1) / sm_count(), fewer = (per_sm + 1) / 2 + 2;
-    if (per_sm > kMostCtas && fewer < kMostCtas) {
-      constexpr int kIds = IDS ? kStages<T, IDS> * kIdSlot * (int)sizeof(int32_t) : 0;
-      const size_t share = ((size_t)kSmSharedBytes / fewer - kCtaSharedBytes - kIds) / 128 * 128;
+    if (per_sm > kMostCtas<T> && per_sm <= kMostEvened) {
+      const size_t share = ((size_t)kSmSharedBytes / fewer - kCtaSharedBytes) / 128 * 128;
       if (share > cfg.dynamicSmemBytes) cfg.dynamicSmemBytes = share;
     }
   }

@@ -496,6 +496,22 @@ def test_offsets_past_32_bits():
     torch.testing.assert_close(grads[3][-3:], g2[3], rtol=1e-3, atol=1e-2)
 
 
+@pytest.mark.parametrize("per_sm", [31, 35, 44, 47])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_long_rows_in_waves(dtype, per_sm):
+    """Long rows, a warp each: the bits do not depend on how many run at a time, with ids or without."""
+    d, L = 148 * per_sm - 5, 8200
+    g = torch.Generator(device="cuda").manual_seed(per_sm)
+    u, r, i = (torch.randn(1, d, L, device="cuda", generator=g).to(dtype) for _ in range(3))
+    A = -torch.rand(d, generator=g, device="cuda")
+    ids = (torch.arange(L, device="cuda") // 1000)[None].to(torch.int32)
+    for seq in (None, ids):
+        whole = mb.gated_linear_scan_fn(u, r, i, A, seq_idx=seq)
+        for s in (slice(0, d // 2), slice(d // 2, d)):
+            # (each half is more rows than 14 an SM, so a warp each too)
+            assert torch.equal(whole[:, s], mb.gated_linear_scan_fn(u[:, s], r[:, s], i[:, s], A[s], seq_idx=seq))
+
+
 def test_opcheck():
     x = cuda(make(2, 5, 300, BF16, initial=True, packed=True))
     ops, utils = torch.ops.mamba_b200, ("test_schema", "test_faketensor")
