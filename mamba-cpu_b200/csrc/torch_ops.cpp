@@ -63,8 +63,20 @@ Tensor make(at::IntArrayRef sizes, const Tensor& like, at::ScalarType t) {
 
 bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
 
+// What the kernels read as float32 is cast on the way there: an imaginary part would be lost.
+void want_real(const char* name, const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.is_complex(), "complex ", name, " is not supported yet");
+}
+
+// The tensor whose type a result takes: results would be cut to integers.
+void want_floating(const char* name, const Tensor& t) {
+  want_real(name, t);
+  TORCH_CHECK_TYPE(t.is_floating_point(), name, " must be of floating point, got ", t.scalar_type());
+}
+
 void want_shape(const char* name, const OptTensor& t, at::IntArrayRef shape, const Tensor& on, const char* on_name) {
   if (!given(t)) return;
+  want_real(name, *t);
   TORCH_CHECK_VALUE(t->sizes() == shape, name, " must be ", shape, ", got ", t->sizes());
   TORCH_CHECK_VALUE(t->device() == on.device(), name, " must be on ", on_name, "'s device ", on.device(), ", got ",
                     t->device());
@@ -243,6 +255,7 @@ at::ScalarType common_io(const Tensor& u, const Tensor& r, const Tensor& i) {
 std::tuple<Tensor, Tensor> gated_scan(const Tensor& u, const Tensor& decay_gate, const Tensor& input_gate,
                                       const Tensor& A, const OptTensor& initial_state, const OptTensor& seq_idx) {
   want_cuda(u);
+  want_floating("u", u);
   TORCH_CHECK_VALUE(u.dim() == 3, "u must be (batch, dim, seqlen), got ", u.sizes());
   const int64_t b = u.size(0), d = u.size(1), l = u.size(2);
   want_shape("decay_gate", decay_gate, u.sizes(), u, "u");
@@ -251,7 +264,6 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& u, const Tensor& decay_gate,
   want_shape("initial_state", initial_state, {b, d}, u, "u");
   want_shape("seq_idx", seq_idx, {b, l}, u, "u");
   no_tangents({&u, &decay_gate, &input_gate, &A}, {&initial_state});
-  TORCH_CHECK_NOT_IMPLEMENTED(!A.is_complex(), "complex A is not supported yet");
   TORCH_CHECK_TYPE(!given(seq_idx) || at::isIntegralType(seq_idx->scalar_type(), /*includeBool=*/false),
                    "seq_idx must hold integers, got ", seq_idx->scalar_type());
   const auto io = common_io(u, decay_gate, input_gate);
@@ -348,15 +360,16 @@ Tensor gated_scan_update_out(const Tensor& state, const Tensor& u, const Tensor&
 Tensor gated_step(Tensor state, const Tensor& u, const Tensor& decay_gate, const Tensor& input_gate, const Tensor& A,
                   OptTensor out_state) {
   want_cuda(u);
+  want_floating("u", u);
   TORCH_CHECK_VALUE(u.dim() == 2, "u must be (batch, dim), got ", u.sizes());
   const int64_t b = u.size(0), d = u.size(1);
   want_shape("state", state, u.sizes(), u, "u");
+  want_floating("state", state);
   want_shape("decay_gate", decay_gate, u.sizes(), u, "u");
   want_shape("input_gate", input_gate, u.sizes(), u, "u");
   want_shape("A", A, {d}, u, "u");
   want_shape("out_state", out_state, u.sizes(), u, "u");
   no_tangents({&state, &u, &decay_gate, &input_gate, &A}, {&out_state});
-  TORCH_CHECK_NOT_IMPLEMENTED(!A.is_complex(), "complex A is not supported yet");
   const bool apart = given(out_state) && !out_state->is_same(state);
   Tensor target = apart ? *out_state : state;
   TORCH_CHECK_TYPE(target.scalar_type() == state.scalar_type(), "out_state must have state's dtype ",
@@ -621,6 +634,7 @@ at::ScalarType weight_type(const OptTensor& w, const OptTensor& b, at::ScalarTyp
 std::tuple<Tensor, Tensor> norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias,
                                 const OptTensor& residual, double eps, bool prenorm, bool residual_in_fp32, bool rms) {
   want_cuda(x);
+  want_floating("x", x);
   TORCH_CHECK_VALUE(x.dim() >= 1, "x must have at least one dimension");
   const int64_t dim = x.size(-1);
   want_shape("weight", weight, {dim}, x, "x");
@@ -654,6 +668,7 @@ std::tuple<Tensor, Tensor> norm(const Tensor& x, const OptTensor& weight, const 
 Tensor gated_norm(const Tensor& x, const Tensor& z, const OptTensor& weight, double eps,
                   std::optional<int64_t> group_size, bool norm_before_gate) {
   want_cuda(x);
+  want_floating("x", x);
   TORCH_CHECK_VALUE(x.dim() >= 1, "x must have at least one dimension");
   const int64_t dim = x.size(-1);
   want_shape("z", z, x.sizes(), x, "x");

@@ -262,6 +262,46 @@ def test_shapes_and_dtypes_on_fake_tensors():
         assert [t.shape for t in got] == [x.shape, (0,), x.shape, (16,), (0,)]
 
 
+_TENSORS = {  # every tensor argument by name, and the call
+    "scan": (dict(u=(2, 4, 8), r=(2, 4, 8), i=(2, 4, 8), A=(4,), h0=(2, 4)),
+             lambda t: mb.gated_linear_scan_fn(t["u"], t["r"], t["i"], t["A"], t["h0"])),
+    "step": (dict(state=(2, 4), u=(2, 4), r=(2, 4), i=(2, 4), A=(4,)),
+             lambda t: mb.gated_linear_scan_update(t["state"], t["u"], t["r"], t["i"], t["A"])),
+    "step to": (dict(state=(2, 4), u=(2, 4), out_state=(2, 4), A=(4,)),
+                lambda t: mb.gated_linear_scan_update(t["state"], t["u"], t["u"], t["u"], t["A"], t["out_state"])),
+    "layer norm": (dict(x=(3, 8), w=(8,), b=(8,), res=(3, 8)),
+                   lambda t: mb.layer_norm_fn(t["x"], t["w"], t["b"], t["res"])),
+    "rms norm": (dict(x=(3, 8), w=(8,), b=(8,), res=(3, 8)),
+                 lambda t: mb.rms_norm_fn(t["x"], t["w"], t["b"], t["res"], prenorm=True)[1]),
+    "gated norm": (dict(x=(3, 8), z=(3, 8), w=(8,)), lambda t: mb.gated_rms_norm_fn(t["x"], t["z"], t["w"])),
+}
+
+
+@pytest.mark.parametrize("name,arg", [(n, a) for n, (shapes, _) in _TENSORS.items() for a in shapes])
+def test_complex_tensors_are_refused(name, arg):
+    """No argument loses its imaginary part on the way to float32."""
+    shapes, call = _TENSORS[name]
+    with FakeTensorMode():
+        t = {k: _fake(*s) for k, s in shapes.items()}
+        t[arg] = _fake(*shapes[arg], dtype=torch.complex64)
+        if arg == "state" and "out_state" in t:
+            t["out_state"] = _fake(*shapes["out_state"], dtype=torch.complex64)
+        with pytest.raises((TypeError, NotImplementedError)):
+            call(t)
+
+
+@pytest.mark.parametrize("name,arg", [("scan", "u"), ("step", "u"), ("step", "state"), ("layer norm", "x"),
+                                      ("rms norm", "x"), ("gated norm", "x")])
+@pytest.mark.parametrize("dtype", [torch.int32, torch.bool])
+def test_results_are_not_cut_to_integers(name, arg, dtype):
+    """The argument whose type a result takes is of floating point."""
+    shapes, call = _TENSORS[name]
+    with FakeTensorMode():
+        t = {k: _fake(*s) for k, s in shapes.items()}
+        with pytest.raises(TypeError, match="floating point"):
+            call({**t, arg: _fake(*shapes[arg], dtype=dtype)})
+
+
 @pytest.mark.parametrize("rms", [False, True])
 @pytest.mark.parametrize("b,l", [(1, 12), (3, 12)])
 def test_mixer_delta_is_read_in_place(monkeypatch, rms, b, l):
@@ -284,21 +324,6 @@ def test_mixer_delta_is_read_in_place(monkeypatch, rms, b, l):
     delta, = seen
     assert y.shape == (b, l, dm) and delta.shape == (b, d, l) and delta.dtype == bf
     assert delta.stride()[1:] == (b * l, 1) and (b == 1 or delta.stride(0) == l)
-
-
-_TENSORS = {  # every tensor argument by name, and the call
-    "scan": (dict(u=(2, 4, 8), r=(2, 4, 8), i=(2, 4, 8), A=(4,), h0=(2, 4)),
-             lambda t: mb.gated_linear_scan_fn(t["u"], t["r"], t["i"], t["A"], t["h0"])),
-    "step": (dict(state=(2, 4), u=(2, 4), r=(2, 4), i=(2, 4), A=(4,)),
-             lambda t: mb.gated_linear_scan_update(t["state"], t["u"], t["r"], t["i"], t["A"])),
-    "step to": (dict(state=(2, 4), u=(2, 4), out_state=(2, 4), A=(4,)),
-                lambda t: mb.gated_linear_scan_update(t["state"], t["u"], t["u"], t["u"], t["A"], t["out_state"])),
-    "layer norm": (dict(x=(3, 8), w=(8,), b=(8,), res=(3, 8)),
-                   lambda t: mb.layer_norm_fn(t["x"], t["w"], t["b"], t["res"])),
-    "rms norm": (dict(x=(3, 8), w=(8,), b=(8,), res=(3, 8)),
-                 lambda t: mb.rms_norm_fn(t["x"], t["w"], t["b"], t["res"], prenorm=True)[1]),
-    "gated norm": (dict(x=(3, 8), z=(3, 8), w=(8,)), lambda t: mb.gated_rms_norm_fn(t["x"], t["z"], t["w"])),
-}
 
 
 @pytest.mark.parametrize("name,arg", [(n, a) for n, (shapes, _) in _TENSORS.items() for a in shapes])
