@@ -16,8 +16,11 @@ import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("MAMBA_B200_LIB", os.path.join(_HERE, "_lib", "libmamba_b200.so"))
-# The torch binding of the ops that are bound in C++ (csrc/torch_ops.cpp).
+# The torch binding of the ops that are bound in C++ (csrc/torch_ops.cpp): the one beside the library or, where a
+# library lies alone, the package's. It needs "libmamba_b200.so" by that name, and the one loaded below has it.
 TORCH_LIB_PATH = os.path.join(os.path.dirname(LIB_PATH), "libmamba_b200_torch.so")
+if not os.path.exists(TORCH_LIB_PATH):
+    TORCH_LIB_PATH = os.path.join(_HERE, "_lib", "libmamba_b200_torch.so")
 
 F32, BF16, F16 = 0, 1, 2
 MAX_DSTATE = 16

@@ -4,7 +4,9 @@ differences."""
 
 import ctypes
 import os
+import shutil
 import subprocess
+import sys
 import tempfile
 
 import numpy as np
@@ -167,6 +169,20 @@ def test_norm_workspace_of_any_alignment(dim):
         p.fwd.x = 0x1000 + off
         assert _lib.lib.mb200_norm_bwd_workspace_size(p) == size
         p.dx, p.fwd.x = 0x1000, 0x1000
+
+
+def test_library_from_another_place():
+    """MAMBA_B200_LIB names a library that lies alone: the package's torch binding loads, and calls that library."""
+    with tempfile.TemporaryDirectory() as td:
+        other = os.path.join(td, "libmamba_b200.so")
+        shutil.copy(os.path.join(os.path.dirname(_lib.__file__), "_lib", "libmamba_b200.so"), other)
+        code = ("import mamba_cpu_b200 as mb, torch; from mamba_cpu_b200 import _lib; torch.ops.mamba_b200.norm.default;"
+                "print(_lib.lib._name); print(*sorted({l.split()[-1] for l in open('/proc/self/maps')"
+                " if 'libmamba_b200.so' in l}))")
+        r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True,
+                           env=dict(os.environ, MAMBA_B200_LIB=other, PYTHONPATH=os.path.join(ROOT, "mamba-cpu_b200")))
+        assert r.returncode == 0, r.stderr
+        assert r.stdout.split() == [other, other]
 
 
 # ---- the public functions on fake CUDA tensors ---------------------------------------------------------
