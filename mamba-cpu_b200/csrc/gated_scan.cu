@@ -245,15 +245,23 @@ __device__ __forceinline__ Marks marks_of(const Ids& x, int t0) {
 
 // ---- joining maps ------------------------------------------------------------------------------------
 
-// Maps h -> A h + B, earlier ones first. With CUT an A of 0 is the start of a sequence: nothing of
-// what came before gets past it, an infinity or a NaN included.
+// Maps h -> A h + B, earlier ones first. Decays are not negative. With CUT an A with its sign bit set has the start
+// of a sequence in it: nothing of what came before gets past it, an infinity or a NaN included. (Not an A of 0: that is
+// also what fast decays, and products of them, underflow to, and they do pass on an infinity or a NaN. A product with
+// a cut in it keeps the sign bit when it underflows.)
+constexpr float kCut = -1.f;
+__device__ __forceinline__ bool is_cut(float A) { return __float_as_int(A) < 0; }
 template <bool CUT>
 __device__ __forceinline__ float apply(float A, float B, float h) {
-  return CUT && A == 0.f ? B : fmaf(A, h, B);
+  return CUT && is_cut(A) ? B : fmaf(A, h, B);
 }
 template <bool CUT>
-__device__ __forceinline__ float times(float A, float before) {
-  return CUT && A == 0.f ? 0.f : A * before;
+__device__ __forceinline__ float times(float A, float before) {  // the map A behind the map `before`
+  return CUT && is_cut(A) ? A : A * before;
+}
+template <bool CUT>
+__device__ __forceinline__ float decay(float A, float v) {  // of a value, which may be negative
+  return CUT && is_cut(A) ? 0.f : A * v;
 }
 
 // Inclusive scan of the lanes' maps: from lane 0 up, or (REVERSE) from lane 31 down.
@@ -430,7 +438,7 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 21 : 6) gated_fwd_kernel(const 
         blank(av, pad, 1.f);
         blank(x, pad, 0.f);
       }
-      if (CUT) blank(av, mk.cut, 0.f);
+      if (CUT) blank(av, mk.cut, kCut);
       float mA = 1.f, mB = 0.f;
 #pragma unroll
       for (int j = 0; j < K; ++j) {
@@ -585,7 +593,7 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 20 : 4) gated_bwd_kernel(const 
         blank(hp, pad, 0.f);
         blank(g, pad, 0.f);
       }
-      if (CUT) blank(av, mk.cut, 0.f);
+      if (CUT) blank(av, mk.cut, kCut);
       // the chunk's states again: hp[j] becomes the state before step j
       float mA = 1.f, mB = 0.f;
 #pragma unroll
@@ -606,7 +614,7 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 20 : 4) gated_bwd_kernel(const 
       // e from the end: the map of a step is e -> a (dy + e)
       mA = whole, mB = 0.f;
 #pragma unroll
-      for (int j = K - 1; j >= 0; --j) mB = times<CUT>(item(av, j), item(g, j) + mB);
+      for (int j = K - 1; j >= 0; --j) mB = decay<CUT>(item(av, j), item(g, j) + mB);
       scan_maps<true, CUT>(lane, mA, mB);
       float e = carry;
       if (NT > 32) {
@@ -620,7 +628,7 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 20 : 4) gated_bwd_kernel(const 
 #pragma unroll
       for (int j = K - 1; j >= 0; --j) {  // g = dy + e; av becomes a g
         item(g, j) += e;
-        e = times<CUT>(item(av, j), item(g, j));
+        e = decay<CUT>(item(av, j), item(g, j));
         item(av, j) = e;
         if (CUT && (mk.cut >> j & 1)) item(hp, j) = 0.f;
       }

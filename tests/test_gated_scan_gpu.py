@@ -167,6 +167,28 @@ def test_a_sequence_keeps_its_infinities():
         assert torch.equal(got[1], ref[1])
 
 
+@pytest.mark.parametrize("b,d,L", [(1, 3, 1000), (3, 1000, 300)])  # rows over several warps, and a warp each
+@pytest.mark.parametrize("A", [-3.0, -40.0, -400.0])
+def test_a_sequence_does_not_lose_its_nan(b, d, L, A):
+    """What is not a number stays so to the end of its sequence, and its gradient to the beginning, however fast the
+    channel forgets: a product of decays that underflows, or a decay that does, is no start of a sequence."""
+    x = make(b, d, L, F32, seed=8)
+    x["A"] = torch.full((d,), A)
+    x["u"][:, 1, 20] = float("nan")
+    x["dy"][:, 2, L - 20] = float("nan")
+    ids = torch.zeros(b, L, dtype=torch.int32)
+    ids[:, 100:120], ids[:, L - 100:] = 1, 2  # marks in the first and the last chunk
+    x["ids"] = ids
+    got, grads = run(x)
+    nan = torch.isnan(got[0]).cpu()
+    want_nan = torch.zeros(b, d, L, dtype=torch.bool)
+    want_nan[:, 1, 20:100] = True
+    assert torch.equal(nan, want_nan)
+    du = torch.zeros(b, d, L, dtype=torch.bool)
+    du[:, 2, L - 100:L - 19] = True
+    assert torch.equal(torch.isnan(grads["u"]).cpu(), du)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_extreme_gates(dtype):
     """Closed and open gates (infinite and at the type's limits), A of 0 and of -200."""
