@@ -14,8 +14,8 @@
 //   du = g m s_i,  d input_gate = g m u s_i (1 - s_i),  d decay_gate = dla A s_r (1 - s_r),  dA = sum dla s_r
 //
 // What bounds it. A step moves 4 elements forward (2 bytes each in bf16: 8 bytes) and 7 backward, and takes
-// 4 special functions forward (two exponentials, a reciprocal and a root; 5 where A < -1: 97 us instead of
-// the 85 below) and 5 backward, of 34 and 60 instructions in all. 8 x 4096 x 2048 bf16:
+// 4 special functions forward (two exponentials, a reciprocal and a root; 5 where A < -1: 98 and
+// 171 us instead of the 85 and 160 below) and 5 backward, of 34 and 60 instructions in all. 8 x 4096 x 2048 bf16:
 // forward 85 us, 6.3 TB/s of 6.55 that a copy reaches, with the special functions 68% busy and 2.9 of 4
 // instructions a cycle issued; backward 160 us, 5.9 TB/s, 2.7 instructions a cycle. 1 x 5120 x 65536:
 // 456 us (5.9 TB/s) and 817 us (5.75). 4 x 2048 x 2048 float32: 42.6 us (6.3) and 76.5 us (6.1). Packed rows

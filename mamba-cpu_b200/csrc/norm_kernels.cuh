@@ -21,7 +21,9 @@
 // 64 us (6.3); backward 131 us (5.1), with 2.3 of 4 instructions a cycle from the 16 warps that its registers
 // leave an SM. Odd widths take half as many instructions again for the ends of rows: 16384 x 4095 gated 101 us
 // (4.0) and 273 (2.5), 65536 x 769 bf16 62 us (3.2) and 117 (2.6). Rows of over 8,192 columns have 64 registers
-// a thread and spill in the backward: 4096 x 16384 with a float32 residual 141 us (5.7) and 344 (3.1).
+// a thread (five of the backward bodies for odd widths are given 32) and spill, 76 to 872 bytes forward and 664 to 1,812
+// backward: 4096 x 16384 with a float32 residual 141 us (5.7) and 300 (3.6), 4096 x 16383, whose rows are read element by
+// element where they do not begin at 16 bytes, 655 (1.2) and 952 (1.1).
 //
 // Rows that are not 16-byte aligned (odd widths) are still moved 16 bytes at a time: a thread's columns
 // begin `phase` columns early, where phase is the row's misalignment, and what the threads at the ends

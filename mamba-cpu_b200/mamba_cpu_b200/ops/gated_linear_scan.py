@@ -52,7 +52,11 @@ def gated_linear_scan_fn(u, decay_gate, input_gate, A, initial_state=None, seq_i
         a_t = exp(A * sigmoid(decay_gate_t))
         h_t = a_t h_{t-1} + sqrt(1 - a_t^2) * sigmoid(input_gate_t) * u_t
 
-    u, decay_gate, input_gate: (batch, dim, seqlen), gates before their sigmoid
+    Every step's input has the factor sqrt(1 - a^2), the first one of a sequence included (there are layers that feed
+    that one without it; scaling u at those steps by the factor's inverse, where it is not 0, gives them).
+
+    u, decay_gate, input_gate: (batch, dim, seqlen), gates before their sigmoid; an input gate below -44, whose
+        sigmoid is under 1e-19, counts as shut
     A: (dim,), not positive: the log of the decay at an open gate (a positive entry gives NaN)
     initial_state: (batch, dim), the state before the first step (zeros if None)
     seq_idx: (batch, seqlen) integers of 32 bits. Packs sequences into a row: a step whose id differs from the one

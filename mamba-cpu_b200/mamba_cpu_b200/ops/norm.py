@@ -45,6 +45,8 @@ def layer_norm_fn(x, weight, bias=None, residual=None, eps=1e-5, prenorm=False, 
     float32; what is normalised is s as held.
     Returns (..., dim) in x's dtype, with prenorm=True also s, the residual of the next block (without a
     residual: x itself, in float32 with residual_in_fp32). Differentiable (once) in every tensor.
+
+    eps is 1e-5 unless given. mamba_ssm's functions of these names take 1e-6: a call ported from there has to say so.
     """
     out, total = _norm(x, weight, bias, residual, eps, prenorm, residual_in_fp32, False)
     return (out, total) if prenorm else out
@@ -65,5 +67,9 @@ def gated_rms_norm_fn(x, z, weight, eps=1e-5, group_size=None, norm_before_gate=
 
     x, z: (..., dim); weight: (dim,) or None; group_size divides dim (default dim) and is at most 16384.
     Returns (..., dim) in x's dtype. Differentiable (once) in x, z and weight.
+
+    The gate comes first unless told otherwise, as in transformers' Mamba-2 mixer, and eps is 1e-5. ``hf.mamba_split_conv1d_scan_combined``, which has
+    mamba_ssm's signature, normalises first and with eps 1e-6 unless told otherwise, and passes both on: calls ported
+    from there have to say norm_before_gate=True and eps=1e-6.
     """
     return _gated_norm(x, z, weight, eps, group_size, norm_before_gate)
